@@ -461,13 +461,6 @@ def _exact_route(state):
             'offsets': offsets.to(torch.int32)}
 
 
-def _power(exponent):
-    """2 ** exponent in 64 bits, exactly (for -200 to 200)."""
-    table = torch.tensor([2.0 ** e for e in range(-200, 201)],
-                         dtype=torch.float64, device=exponent.device)
-    return table[exponent.long() + 200]
-
-
 def _exact_codec(x):
     """Each value's nearest neighbour on its block's grid, in 64 bits."""
     x = x.double()
@@ -481,8 +474,8 @@ def _exact_codec(x):
         peak = part.abs().amax(1, keepdim=True)
         power = torch.floor(torch.log2(peak.clamp(min=2.0 ** -160)))
         # log2 may round up to a whole number just below a power of two
-        power = power - (_power(power) > peak).double()
-        step = _power((power - 2).clamp(min=-127.0))
+        power = power - (torch.pow(2.0, power) > peak).double()
+        step = torch.pow(2.0, (power - 2).clamp(min=-127.0))
         nearest = (part.abs().unsqueeze(-1) / step.unsqueeze(-1)
                    - grid).abs().argmin(-1)
         out[start:start + (1 << 18)] = torch.copysign(grid[nearest] * step,
@@ -496,9 +489,9 @@ def _exact_values(codes, scales):
     exponent, mantissa = (fields >> 1) & 3, (fields & 1).double()
     magnitude = torch.where(exponent == 0, mantissa * 0.5,
                             (1 + mantissa / 2)
-                            * _power(exponent - 1))
+                            * torch.pow(2.0, exponent.double() - 1))
     sign = 1.0 - 2.0 * (fields >> 3).double()
-    scale = _power(scales.int() - 127)
+    scale = torch.pow(2.0, scales.double() - 127)
     return sign * magnitude * scale.repeat_interleave(BLOCK, -1)
 
 
