@@ -29,9 +29,11 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) unsigned scale4_t;
 
 // Matrix instructions on AGPR accumulators (with the builtins the operands
-// land in AGPRs and VGPRs spill).  Operands come from LDS reads, for which the
-// compiler waits, and VALU results; the epilogue's first read of an
-// accumulator waits in drain().  Byte `S` of both scale registers.
+// land in AGPRs and VGPRs spill).  Inline asm gets no wait states: operands
+// come from LDS reads, for which the compiler waits; scales, which VALU
+// instructions pack, are held to their place before a barrier (settle), for a
+// matrix instruction needs two wait states behind them; the epilogue's first
+// read of an accumulator waits in drain().  Byte `S` of both scale registers.
 template <int S>
 __device__ __forceinline__ void mfma_mx(f32x16& acc, const i32x4& w,
                                         const i32x4& x, int ws, int xs) {
@@ -47,6 +49,15 @@ __device__ __forceinline__ void mfma_mx_first(f32x16& acc, const i32x4& w,
                "op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
                : "=a"(acc)
                : "v"(w), "v"(x), "v"(ws), "v"(xs));
+}
+
+// No VALU instruction that makes these words is moved behind this point.
+template <int N>
+__device__ __forceinline__ void settle(int (&words)[N][4]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(words[k][q]));
 }
 
 // Lane l holds product row l & 31 and columns 8 b + 4 (l >> 5) .. + 3 of a
@@ -299,6 +310,8 @@ __device__ __forceinline__ void run_tile(const ProductArgs& p, const Work& w,
 #pragma unroll
         for (int k = 0; k < TN; ++k) ws[k][q] = ws_next[k][q];
       }
+      settle(xs);
+      settle(ws);
     }
   };
 
@@ -311,6 +324,8 @@ __device__ __forceinline__ void run_tile(const ProductArgs& p, const Work& w,
   for (int k = 0; k < 4; ++k) pack(0, ta[k], xs[k]);
 #pragma unroll
   for (int k = 0; k < TN; ++k) pack(0, tb[k], ws[k]);
+  settle(xs);
+  settle(ws);
   __builtin_amdgcn_s_waitcnt(wait_imm(kA + kB));
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);

@@ -69,6 +69,16 @@ def _run(cmd, verbose):
     return proc.stdout
 
 
+def device_flags():
+    """hipcc flags of every HIP unit."""
+    return ['-O3', '-std=c++17', '-fPIC', '--offload-arch=' + ARCH,
+            '-Wall', '-Wno-unused-result', '-Wno-unused-function',
+            # no packed fp32 arithmetic: some of its forms have given wrong
+            # results on MI355X (the host pass ignores the feature)
+            '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
+            '-fvisibility=hidden'] + _includes()
+
+
 def compile_units(verbose=False, jobs=4):
     os.makedirs(OBJ, exist_ok=True)
     headers = _headers(os.path.join(ROOT, 'csrc'))
@@ -78,12 +88,7 @@ def compile_units(verbose=False, jobs=4):
         for name in sorted(os.listdir(d)):
             if name.endswith(('.hip', '.cpp')):
                 units.append(os.path.join(d, name))
-    flags = ['-O3', '-std=c++17', '-fPIC', '--offload-arch=' + ARCH,
-             '-Wall', '-Wno-unused-result', '-Wno-unused-function',
-             # no packed fp32 arithmetic: some of its forms have given wrong
-             # results on MI355X (the host pass ignores the feature)
-             '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
-             '-fvisibility=hidden'] + _includes()
+    flags = device_flags()
     jobs_list = []
     for src in units:
         obj = os.path.join(OBJ, os.path.basename(src) + '.o')
