@@ -11,10 +11,13 @@ Two start modes (both spawned by :mod:`kiosk_autoscaler_amd.gpumgr`):
   as ``standby_gpu_s``); with deep idle (``POOL_IDLE_RELEASE_S``) only from
   just before the tick that assigns it until just after its scale-down.
   Report ``standby`` and block on the command pipe.
-* **cold** (``--assign JSON``): start immediately.  The HIP context and
-  the code objects are created on a helper thread (``preinit_device``
-  releases the GIL) while the main thread imports the runtime and connects
-  to Redis; the engine joins it.
+* **cold** (``--assign JSON``): start immediately.  In a process that the
+  zygote forked, with its imports done, the HIP context and the code objects
+  are created on a helper thread (``preinit_device`` releases the GIL) while
+  the main thread connects to Redis; the engine joins it.  A process started
+  by itself opens the device on its main thread, as a standby does: one such
+  worker, opening it on the helper thread beside its imports, once ended with
+  SIGSEGV before READY, and the cause is not known.
 
 With the node communicator (``node_fence`` in the pin/assignment) the
 process also runs a :class:`~..parallel.nodefence.NodeFenceAgent` for its
@@ -124,7 +127,8 @@ def _preimport(backend):
             pass   # the assignment reports it, as a failed start
 
 
-# cold spawn: the helper thread opening the device (see the module doc)
+# cold spawn: the helper thread opening the device, or the call that does it
+# when the engine asks (see the module doc)
 _DEVICE_OPEN = {}
 
 
@@ -178,29 +182,39 @@ def _bind_device(mod):
         mod.set_device(device_ordinal())
 
 
-def _open_device_async():
+def _open_device():
+    """Create the HIP context and load the code objects."""
     from ..ops import native
     from .pinning import device_ordinal
-    mod = native.load()
+    try:
+        _DEVICE_OPEN['stages'] = dict(native.load().preinit_device(
+            device_ordinal()))
+        _DEVICE_OPEN['stages'].update(_warm_torch())
+    except Exception as err:  # pylint: disable=broad-except
+        # the engine's own init reports the failure
+        _DEVICE_OPEN['error'] = str(err)
 
-    def run():
-        try:
-            _DEVICE_OPEN['stages'] = dict(mod.preinit_device(
-                device_ordinal()))
-            _DEVICE_OPEN['stages'].update(_warm_torch())
-        except Exception as err:  # pylint: disable=broad-except
-            # the engine's own init reports the failure
-            _DEVICE_OPEN['error'] = str(err)
-    thread = threading.Thread(target=run, name='device-open', daemon=True)
+
+def _open_device_async():
+    from ..ops import native
+    native.load()
+    thread = threading.Thread(target=_open_device, name='device-open',
+                              daemon=True)
     _DEVICE_OPEN['thread'] = thread
     thread.start()
 
 
 def _join_device_open(stage=None):
+    """The device is open behind this (without ``stage``, at the process's
+    end: nothing is opening it)."""
     thread = _DEVICE_OPEN.pop('thread', None)
-    if thread is None:
+    later = _DEVICE_OPEN.pop('later', None)
+    if thread is not None:
+        thread.join()
+    elif later is not None and stage:
+        later()
+    else:
         return
-    thread.join()
     if 'error' not in _DEVICE_OPEN:
         from ..ops import native
         _bind_device(native.load())
@@ -388,7 +402,8 @@ def _build_fence_factory(config):
     return make_agent_factory(config)
 
 
-def main(argv=None):
+def main(argv=None, forked=False):
+    """``forked``: by the zygote, which has done the imports."""
     parser = argparse.ArgumentParser(description=__doc__)
     parser.add_argument('--cmd-fd', type=int, default=None)
     parser.add_argument('--ev-fd', type=int, default=None)
@@ -404,8 +419,8 @@ def main(argv=None):
         return _standalone(args.backend)
     _die_with_parent()
     _stack_dump_on_sigusr1()
-    # ordered for the cold spawn: pin, load the native module and start
-    # opening the device first; logging, the channel and the runtime
+    # ordered for the forked cold spawn: pin, load the native module and
+    # start opening the device first; logging, the channel and the runtime
     # modules load while the helper thread creates the HIP context
     from .pinning import apply_assignment_env, parse_assignment
     backend = args.backend
@@ -431,7 +446,10 @@ def main(argv=None):
                               'visible': early.get('visible')})
     preload_ns = _preload(backend)
     if args.assign and backend == 'hip':
-        _open_device_async()
+        if forked:
+            _open_device_async()
+        else:
+            _DEVICE_OPEN['later'] = _open_device
     if pin and not args.assign and backend == 'hip' and \
             pin.get('preinit') == 'device' and pin.get('node_fence') and \
             os.environ.get('FENCE', 'auto') in ('auto', 'rccl'):

@@ -21,7 +21,7 @@ Protocol (manager <-> zygote, one ``AF_UNIX`` ``SOCK_SEQPACKET`` pair):
   late answer to one the manager gave up on, and is dropped.
 
 The worker process then runs :func:`kiosk_autoscaler_amd.worker.main.main`
-with the same argv a ``subprocess`` spawn would have used.
+with the same argv a ``subprocess`` spawn would have used (and ``forked``).
 """
 import itertools
 import json
@@ -321,7 +321,7 @@ def _child(request, fds, sock):
     sys.argv = ['kiosk-worker'] + argv
     from . import main as worker_main
     try:
-        code = worker_main.main(argv)
+        code = worker_main.main(argv, forked=True)
     except SystemExit as stop:
         code = stop.code if isinstance(stop.code, int) else 1
     except BaseException:  # pylint: disable=broad-except

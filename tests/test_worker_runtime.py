@@ -125,6 +125,90 @@ def test_cold_spawn_opens_the_device_on_a_helper_thread(monkeypatch):
     worker_main._DEVICE_OPEN.clear()
 
 
+COLD = """
+import os, sys, threading
+from kiosk_autoscaler_amd.ops import native
+from kiosk_autoscaler_amd.worker import main as worker_main
+
+
+class Mod(object):
+    def preinit_device(self, device):
+        print('opened on', threading.current_thread().name, flush=True)
+        return {'preinit_done': 1}
+
+    def release_kept_stream(self):
+        pass
+
+
+class Runtime(object):
+    recycle, keys_done = False, 0
+
+
+def serve(assignment, backend, channel, node_agent=None):
+    print('serving', flush=True)
+    if sys.argv[2] == 'engine':
+        worker_main._join_device_open(
+            lambda name, t=None: print(name, flush=True))
+    return 0, Runtime()
+
+
+native.load = lambda **kw: Mod()
+worker_main._serve = serve
+worker_main.main(['--backend', 'hip', '--assign', '{"gpu": "0"}'],
+                 **eval(sys.argv[1]))
+"""
+
+
+@pytest.mark.parametrize('how,engine,want', [
+    ({'forked': True}, 'engine',
+     ['opened on device-open', 'serving', 'preinit_done',
+      'device_open_joined']),
+    ({}, 'engine', ['serving', 'opened on MainThread', 'preinit_done',
+                    'device_open_joined']),
+    # an assignment that ends before its engine opens nothing
+    ({}, 'none', ['serving'])])
+def test_only_a_forked_worker_opens_the_device_on_a_helper_thread(
+        how, engine, want):
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run(
+        [sys.executable, '-c', COLD, repr(how), engine], text=True,
+        capture_output=True, timeout=60, cwd=root,
+        env=dict(os.environ, FENCE='none', PYTHONPATH=root))
+    lines = done.stdout.split('\n')[:-1]
+    # (beside the main thread's own steps the helper thread may be late)
+    assert (sorted(lines) if how else lines) == \
+        (sorted(want) if how else want), (lines, done.stderr)
+
+
+def test_zygote_tells_the_worker_that_it_is_forked(monkeypatch):
+    import socket
+    from kiosk_autoscaler_amd.worker import main as worker_main
+    from kiosk_autoscaler_amd.worker import zygote
+    calls = []
+
+    class Ended(Exception):
+        pass
+
+    def end(code):
+        raise Ended
+    monkeypatch.setattr(worker_main, 'main',
+                        lambda argv, **kw: calls.append((argv, kw)) or 0)
+    monkeypatch.setattr(os, '_exit', end)
+    monkeypatch.setattr(os, 'setsid', lambda: None)
+    monkeypatch.setattr(os, 'close', lambda fd: None)
+    monkeypatch.setattr(zygote.signal, 'signal', lambda *a: None)
+    monkeypatch.setattr(os, 'environ', dict(os.environ))
+    monkeypatch.setattr('sys.argv', ['x'])
+    ours, theirs = socket.socketpair()
+    with pytest.raises(Ended):
+        zygote._child({'env': {}, 'argv': ['--backend', 'hip']}, (7, 8),
+                      theirs)
+    ours.close()
+    assert calls == [(['--backend', 'hip'], {'forked': True})]
+
+
 class _FenceAgent(object):
     def __init__(self):
         self.calls = []
