@@ -3,15 +3,15 @@
 The fence ``dlopen``s RCCL (``csrc/runtime/fence.cpp``, ``KIOSK_RCCL_LIB``),
 by default ROCm's installed ``librccl.so.1`` as it is.
 
-An operator who builds RCCL from source names the build with
-``KIOSK_RCCL_SRC``.  A build for several GPU targets carries their device
+An operator who builds RCCL from source may load the build as it is
+(``KIOSK_RCCL_LIB``) or name it with ``KIOSK_RCCL_SRC``.  A build for several GPU targets carries their device
 code in one zstd-compressed offload bundle, which the HIP runtime inflates
 whole in the first ``ncclCommInitRank`` of each process;
 :func:`ensure_slim` writes, once per host and build, a copy that holds only
 the gfx950 code object, uncompressed and without its DWARF
 (``build/kiosk-rccl-slim``, ``csrc/tools/rccl_slim.cpp``).  The manager
 calls it at start and points its workers at the copy (``RCCL_SLIM``, default
-on where a build is named).  The copy lives in a cache directory
+on where a build is named); without a copy they load ROCm's library.  The copy lives in a cache directory
 (``KIOSK_CACHE_DIR``, default ``~/.cache/kiosk-autoscaler-amd``) beside a
 ``share/rccl`` link, so RCCL still finds its MSCCL algorithm files relative
 to itself.
@@ -47,9 +47,8 @@ def cache_root(env=None):
 
 
 def source_library(env=None):
-    """The RCCL workers load without a slim copy: the operator's build
-    (``KIOSK_RCCL_SRC``), else ROCm's (its ``ncclCommShrink`` is what the
-    node communicator needs)."""
+    """What the slim copy is made from, and what the library ladder goes
+    back to: the operator's build (``KIOSK_RCCL_SRC``), else ROCm's."""
     env = os.environ if env is None else env
     return os.path.realpath(env.get('KIOSK_RCCL_SRC') or STOCK)
 
@@ -186,7 +185,8 @@ def configure(env=None, isa=None, log=None):
     unless ``KIOSK_RCCL_LIB`` already names a library or ``RCCL_SLIM=0``,
     make (or find) the slim copy and export it as ``KIOSK_RCCL_LIB`` into
     ``env`` (default ``os.environ``), which every zygote, standby and worker
-    inherits.  Returns the info dict."""
+    inherits.  Where no copy is made nothing is exported: workers load
+    ROCm's library.  Returns the info dict."""
     env = os.environ if env is None else env
     log = log or logger
     if env.get('KIOSK_RCCL_LIB'):
@@ -201,7 +201,8 @@ def configure(env=None, isa=None, log=None):
     path, info = ensure_slim(isa=isa, env=env)
     if path is None:
         log.warning('slim RCCL unavailable (%s): workers load the stock '
-                    'library.', info.get('error'))
+                    'library (KIOSK_RCCL_LIB names another).',
+                    info.get('error'))
         return dict(info, lib=None, slim=False)
     env['KIOSK_RCCL_LIB'] = path
     log.info('RCCL for the node communicator: %s (%s, %.0f ms%s).', path,

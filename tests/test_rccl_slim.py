@@ -406,6 +406,27 @@ def test_configure_falls_back_to_stock_without_the_tool(tmp_path):
     assert out.get('error')
 
 
+def test_a_build_that_is_not_copied_is_loaded_only_by_name(tmp_path):
+    """A build that the tool refuses: the stock library, with a warning that
+    says how the build itself is loaded."""
+    lib = tmp_path / 'librccl.so.1'
+    lib.write_bytes(b'no library')
+    env = {'KIOSK_CACHE_DIR': str(tmp_path / 'cache'),
+           'KIOSK_RCCL_SRC': str(lib)}
+    lines = []
+
+    class Log(object):
+        @staticmethod
+        def warning(text, *args):
+            lines.append(text % args)
+    out = rccl_lib.configure(env=env, log=Log)
+    assert out['lib'] is None and out['slim'] is False and out['error']
+    assert 'KIOSK_RCCL_LIB' not in env
+    assert 'stock library' in lines[0] and 'KIOSK_RCCL_LIB' in lines[0]
+    env['KIOSK_RCCL_LIB'] = str(lib)
+    assert rccl_lib.configure(env=env)['lib'] == str(lib)
+
+
 INSTALLED = ('an installed library is compiled code that was not built here: '
              'it is no longer taken apart (only a KIOSK_RCCL_SRC build is)')
 
