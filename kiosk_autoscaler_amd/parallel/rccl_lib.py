@@ -4,17 +4,17 @@ The fence ``dlopen``s RCCL (``csrc/runtime/fence.cpp``, ``KIOSK_RCCL_LIB``),
 by default ROCm's installed ``librccl.so.1`` as it is.
 
 An operator who builds RCCL from source may load the build as it is
-(``KIOSK_RCCL_LIB``) or name it with ``KIOSK_RCCL_SRC``.  A build for several GPU targets carries their device
-code in one zstd-compressed offload bundle, which the HIP runtime inflates
-whole in the first ``ncclCommInitRank`` of each process;
-:func:`ensure_slim` writes, once per host and build, a copy that holds only
-the gfx950 code object, uncompressed and without its DWARF
-(``build/kiosk-rccl-slim``, ``csrc/tools/rccl_slim.cpp``).  The manager
-calls it at start and points its workers at the copy (``RCCL_SLIM``, default
-on where a build is named); without a copy they load ROCm's library.  The copy lives in a cache directory
-(``KIOSK_CACHE_DIR``, default ``~/.cache/kiosk-autoscaler-amd``) beside a
-``share/rccl`` link, so RCCL still finds its MSCCL algorithm files relative
-to itself.
+(``KIOSK_RCCL_LIB``) or name it with ``KIOSK_RCCL_SRC``.  A build for several
+GPU targets carries their device code in one zstd-compressed offload bundle,
+which the HIP runtime inflates whole in the first ``ncclCommInitRank`` of each
+process; :func:`ensure_slim` writes, once per host and build, a copy that
+holds only the gfx950 code object, uncompressed and without its DWARF
+(``build/kiosk-rccl-slim``, ``csrc/tools/rccl_slim.cpp``).  The manager calls
+it at start and points its workers at the copy (``RCCL_SLIM``, default on
+where a build is named); without a copy they load ROCm's library.  The copy
+lives in a cache directory (``KIOSK_CACHE_DIR``, default
+``~/.cache/kiosk-autoscaler-amd``) beside a ``share/rccl`` link, so RCCL still
+finds its MSCCL algorithm files relative to itself.
 
 Only such a build is taken apart: an installed library is compiled code
 that was not built here, so :func:`ensure_slim` and the tool refuse it.
