@@ -12,11 +12,28 @@ def device_of(t, name):
     return t.device
 
 
+class _Forward(object):
+    """Stands for torch's forward_ad until the first call: inside a level."""
+    _current_level = 0
+
+
+_FORWARD = _Forward
+
+
+def tangent(t):
+    """Whether ``t`` is a dual tensor of forward-mode differentiation."""
+    global _FORWARD  # pylint: disable=global-statement
+    if _FORWARD is _Forward:
+        from torch.autograd import forward_ad as _FORWARD
+    return _FORWARD._current_level >= 0 and \
+        _FORWARD.unpack_dual(t).tangent is not None
+
+
 def tensor(t, name, dtypes, device=None, shape=None, dims=None, align=16):
     """Refuse a tensor that a kernel cannot take: another device, type or
     shape, holes between its elements, an address that is not a multiple of
-    ``align`` bytes, or one whose gradient would be lost.  ``dtypes``: a type
-    or a tuple of them."""
+    ``align`` bytes, or one whose gradient or tangent would be lost.
+    ``dtypes``: a type or a tuple of them."""
     where = t.device if getattr(t, 'is_cuda', False) else device_of(t, name)
     dtype = t.dtype
     if dtype is not dtypes and not (isinstance(dtypes, tuple)
@@ -44,6 +61,11 @@ def tensor(t, name, dtypes, device=None, shape=None, dims=None, align=16):
         if torch.is_grad_enabled():
             raise ValueError('%s requires a gradient: these operators have '
                              'no backward pass (use torch.no_grad())' % name)
+    # (outside every level one comparison, 0.03 us)
+    if _FORWARD._current_level >= 0 and tangent(t):
+        raise ValueError('%s has a tangent: these operators have no '
+                         'derivative (forward_ad.unpack_dual gives the '
+                         'tensor without it)' % name)
     return where
 
 

@@ -16,7 +16,7 @@ Each call runs hand-written HIP kernels on the operands' device, on the
 caller's current stream there.  Memory beside the operands comes from torch's
 allocator: the result and, for :func:`grouped_gemm` of many rows, a workspace;
 a call that is given both (a capture that torch does not know of) allocates
-nothing.  There is no backward pass.
+nothing.  There is no backward pass and no forward-mode derivative.
 """
 import collections
 import functools

@@ -399,6 +399,33 @@ def test_mxfp4_refuses(host):
             mxfp4.gemm(**dict(dict(a=a, b=b), **call))
 
 
+def test_dual_tensors_are_refused(host):
+    """A tangent would be lost without a word."""
+    forward = torch.autograd.forward_ad
+    f32, off = torch.float32, zeros(2, dtype=torch.int32)
+    calls = {
+        'logits': lambda t: experts.route(t, 1),
+        'a': lambda t: experts.grouped_gemm(t, zeros(1, 16, 64), off),
+        'b': lambda t: experts.grouped_gemm(zeros(2, 64),
+                                            t.view(1, 16, 64), off),
+        'bias': lambda t: mxfp4.gemm(mx_zeros(2, 128), mx_zeros(16, 128),
+                                     bias=t, epilogue='bias'),
+        'y': lambda t: experts.combine(t, zeros(2, 1, dtype=torch.int32),
+                                       zeros(2, 1, dtype=f32)),
+        'x': mxfp4.quantize}
+    for name, call in calls.items():
+        t = {'b': zeros(16, 64), 'bias': zeros(16, dtype=f32)}.get(
+            name, zeros(2, 64))
+        with forward.dual_level():
+            with pytest.raises(ValueError, match=name + ' has a tangent'):
+                call(forward.make_dual(t, torch.ones_like(t)))
+            # a tensor without one passes within the level too
+            with pytest.raises(AssertionError, match='launched'):
+                call(t)
+        with pytest.raises(AssertionError, match='launched'):
+            call(t)
+
+
 # ---------------------------------------------------------------------------
 # numerics
 
