@@ -62,7 +62,7 @@ struct ProductArgs {
   const uint8_t* b_scales;
   uint16_t* c;
   const float* bias;          // [experts, n]
-  const uint16_t* residual;   // [rows_c, n]
+  const uint16_t* residual;   // [rows_c, n], MXFP4 only
   const int* offsets;         // [experts + 1], null: one group of all rows
   const int* rows;            // [rows_c] gather, null: row i of a
   int rows_a, rows_c, n, row_bytes, experts;

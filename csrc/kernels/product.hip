@@ -202,7 +202,8 @@ template <int MODE>
 hipError_t configure_mode() {
   hipError_t err = configure<MODE, PRODUCT_NONE>();
   if (err == hipSuccess) err = configure<MODE, PRODUCT_BIAS_GELU>();
-  if (err == hipSuccess) err = configure<MODE, PRODUCT_BIAS_RESIDUAL>();
+  if constexpr (MODE == kMx)
+    if (err == hipSuccess) err = configure<MODE, PRODUCT_BIAS_RESIDUAL>();
   if (err == hipSuccess) err = configure<MODE, PRODUCT_BIAS>();
   return err;
 }
@@ -235,10 +236,11 @@ hipError_t launch_mode(const ProductArgs& p, hipStream_t stream) {
       return launch_epilogue<MODE, PRODUCT_NONE>(p, stream);
     case PRODUCT_BIAS_GELU:
       return launch_epilogue<MODE, PRODUCT_BIAS_GELU>(p, stream);
-    case PRODUCT_BIAS_RESIDUAL:
-      return launch_epilogue<MODE, PRODUCT_BIAS_RESIDUAL>(p, stream);
     case PRODUCT_BIAS:
       return launch_epilogue<MODE, PRODUCT_BIAS>(p, stream);
+    case PRODUCT_BIAS_RESIDUAL:
+      if constexpr (MODE == kMx)
+        return launch_epilogue<MODE, PRODUCT_BIAS_RESIDUAL>(p, stream);
     default:
       return hipErrorInvalidValue;
   }
@@ -311,7 +313,9 @@ hipError_t launch_product(const ProductArgs& p, hipStream_t stream) {
       (p.offsets == nullptr && p.experts != 1) ||
       (p.a_scales == nullptr) != (p.b_scales == nullptr) ||
       (p.epilogue != PRODUCT_NONE && p.bias == nullptr) ||
-      (p.epilogue == PRODUCT_BIAS_RESIDUAL && p.residual == nullptr))
+      // (the bf16 product with a residual is gemm's)
+      (p.epilogue == PRODUCT_BIAS_RESIDUAL &&
+       (p.residual == nullptr || p.a_scales == nullptr)))
     return hipErrorInvalidValue;
   switch (pick(p)) {
     case kRows:

@@ -399,6 +399,24 @@ def test_mxfp4_refuses(host):
             mxfp4.gemm(**dict(dict(a=a, b=b), **call))
 
 
+def test_only_the_kernels_that_calls_reach_are_built():
+    """No bf16 product takes a residual (gemm does): none is compiled."""
+    paths = native.extension_candidates()
+    if not paths:
+        pytest.skip('the extension is not built')
+    with open(paths[0], 'rb') as f:
+        built = f.read()
+    for name in (b'product_tile_kernel', b'product256_bf16_kernel',
+                 b'product_rows_kernel'):
+        assert name + b'ILi' in built
+    # <mode 0 (bf16), epilogue 2 (residual), ...>
+    for name in (b'product_tile_kernelILi0ELi2E',
+                 b'product256_bf16_kernelILi2E',
+                 b'product_rows_kernelILi0ELi2E'):
+        assert name not in built
+    assert b'product_tile_kernelILi1ELi2E' in built
+
+
 def test_dual_tensors_are_refused(host):
     """A tangent would be lost without a word."""
     forward = torch.autograd.forward_ad
@@ -1044,6 +1062,25 @@ def test_calls_on_two_streams_at_once(mx):
     torch.cuda.synchronize()
     for out, want in got:
         assert torch.equal(out, want)
+
+
+@gpu
+@pytest.mark.parametrize('m,n,k', [(4, 512, 512), (512, 512, 1024),
+                                   (1500, 1024, 4096)])
+def test_a_bf16_residual_is_refused_by_the_binding(m, n, k):
+    """Whatever tile the size picks: an error, nothing launched."""
+    mod = native.load()
+    a, b, out = rand(m, k), rand(n, k), rand(m, n, seed=2)
+    bias = rand(n, dtype=torch.float32)
+    offsets = torch.tensor([0, m], dtype=torch.int32, device='cuda')
+    want = out.clone()
+    with pytest.raises(RuntimeError, match='invalid'):
+        mod.product(a.data_ptr(), 0, b.data_ptr(), 0, out.data_ptr(),
+                    bias.data_ptr(), out.data_ptr(), offsets.data_ptr(), 0,
+                    m, m, n, 2 * k, 1, 2, False, 256, 0,
+                    torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
 
 
 @gpu
