@@ -71,10 +71,12 @@ struct ProductArgs {
   int cus;                    // compute units of the device
   float* partial;             // workspace (product_workspace bytes) or null
   int pieces;                 // partial tiles that it holds (set by launch)
+  bool dry;                   // check the sizes, launch nothing
 };
 // Bytes of fp32 workspace that speed the product up (0: none is used).  Only
 // the sizes, `cus` and whether scales, offsets and rows are null matter.
 size_t product_workspace(const ProductArgs& args);
+// hipErrorInvalidConfiguration: more tiles than one launch takes.
 hipError_t launch_product(const ProductArgs& args, hipStream_t stream);
 hipError_t experts_prepare();   // load the code objects, raise LDS limits
 

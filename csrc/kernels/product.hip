@@ -218,15 +218,14 @@ hipError_t launch_epilogue(const ProductArgs& p, hipStream_t stream) {
   const int tiles_m = most_tiles(p.rows_c, p.experts, BM);
   const int tiles_n = (p.n + BN - 1) / BN;
   const long long blocks = tiles128(p) + (p.zero_rest ? kZeroBlocks : 0);
-  if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(blocks)), block(kThreads);
   // a tile for each CU: deep; two of them there hide each other's waits
   return tiles128(p) <= p.cus
-             ? launch_kernel(&product_tile_kernel<MODE, EPI, 4>, grid, block,
-                             4 * kStepBytes<MODE>, stream, p, tiles_m, tiles_n)
-             : launch_kernel(&product_tile_kernel<MODE, EPI, 2>, grid, block,
-                             2 * kStepBytes<MODE>, stream, p, tiles_m,
-                             tiles_n);
+             ? launch_tiles(&product_tile_kernel<MODE, EPI, 4>, blocks,
+                            kThreads, 4 * kStepBytes<MODE>, stream, p, tiles_m,
+                            tiles_n)
+             : launch_tiles(&product_tile_kernel<MODE, EPI, 2>, blocks,
+                            kThreads, 2 * kStepBytes<MODE>, stream, p, tiles_m,
+                            tiles_n);
 }
 
 template <int MODE>

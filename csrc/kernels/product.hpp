@@ -6,6 +6,7 @@
 
 #include "common.hpp"
 #include "experts.hpp"
+#include "launch.hpp"
 
 namespace kiosk {
 
@@ -194,6 +195,18 @@ __host__ __device__ inline int most_tiles(int rows, int experts, int bm) {
                       : rows / bm + (experts < rows ? experts : rows);
 }
 
+// Launches the first kernel of a product, if its grid is within bounds: fewer
+// than 2^32 threads.
+template <typename Kernel, typename... Args>
+hipError_t launch_tiles(Kernel kernel, long long blocks, int threads,
+                        unsigned lds, hipStream_t stream,
+                        const ProductArgs& p, Args... args) {
+  if (blocks > 0xffffffffll / threads) return hipErrorInvalidConfiguration;
+  if (p.dry) return hipSuccess;
+  return launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)),
+                       dim3(threads), lds, stream, p, args...);
+}
+
 // product256.hip
 bool product256_ok(const ProductArgs& p);
 size_t product256_workspace(const ProductArgs& p);
@@ -203,9 +216,9 @@ hipError_t launch_product256(const ProductArgs& p, hipStream_t stream);
 hipError_t product256_bf16_prepare();
 hipError_t product256_mx_prepare();
 hipError_t launch_product256_bf16(const ProductArgs& p, int tiles_n, int grid,
-                                  int blocks, hipStream_t stream);
+                                  long long blocks, hipStream_t stream);
 hipError_t launch_product256_mx(const ProductArgs& p, int tiles_n, int grid,
-                                int blocks, hipStream_t stream);
+                                long long blocks, hipStream_t stream);
 // product_rows.hip
 hipError_t launch_product_rows(const ProductArgs& p, hipStream_t stream);
 

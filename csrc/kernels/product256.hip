@@ -78,12 +78,11 @@ hipError_t launch_product256(const ProductArgs& args, hipStream_t stream) {
       static_cast<long long>(most_tiles(p.rows_c, p.experts, BM)) * tiles_n +
       pieces;
   const long long blocks = grid + (p.zero_rest ? kZeroBlocks : 0);
-  if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
+  // (`grid` fits 32 bits where `blocks` is launched)
   const hipError_t err =
       (p.a_scales != nullptr ? launch_product256_mx : launch_product256_bf16)(
-          p, tiles_n, static_cast<int>(grid), static_cast<int>(blocks),
-          stream);
-  if (err != hipSuccess || pieces == 0) return err;
+          p, tiles_n, static_cast<int>(grid), blocks, stream);
+  if (err != hipSuccess || pieces == 0 || p.dry) return err;
   switch (p.epilogue) {
     case PRODUCT_BIAS_GELU:
       return join<PRODUCT_BIAS_GELU>(p, tiles_n, pieces, stream);

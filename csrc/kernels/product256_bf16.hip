@@ -234,10 +234,10 @@ hipError_t product256_bf16_prepare() {
 }
 
 hipError_t launch_product256_bf16(const ProductArgs& p, int tiles_n, int grid,
-                                  int blocks, hipStream_t stream) {
+                                  long long blocks, hipStream_t stream) {
   auto launch = [&](auto kernel) {
-    return launch_kernel(kernel, dim3(blocks), dim3(kThreads), kLdsBytes,
-                         stream, p, tiles_n, grid);
+    return launch_tiles(kernel, blocks, kThreads, kLdsBytes, stream, p, tiles_n,
+                        grid);
   };
   switch (p.epilogue) {
     case PRODUCT_NONE:

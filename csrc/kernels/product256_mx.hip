@@ -399,11 +399,11 @@ hipError_t configure_all() {
 }
 
 template <bool CUT>
-hipError_t launch_cut(const ProductArgs& p, int tiles_n, int grid, int blocks,
-                      hipStream_t stream) {
+hipError_t launch_cut(const ProductArgs& p, int tiles_n, int grid,
+                      long long blocks, hipStream_t stream) {
   auto launch = [&](auto kernel) {
-    return launch_kernel(kernel, dim3(blocks), dim3(kThreads), kLdsBytes,
-                         stream, p, tiles_n, grid);
+    return launch_tiles(kernel, blocks, kThreads, kLdsBytes, stream, p, tiles_n,
+                        grid);
   };
   switch (p.epilogue) {
     case PRODUCT_NONE:
@@ -427,7 +427,7 @@ hipError_t product256_mx_prepare() {
 }
 
 hipError_t launch_product256_mx(const ProductArgs& p, int tiles_n, int grid,
-                                int blocks, hipStream_t stream) {
+                                long long blocks, hipStream_t stream) {
   return p.row_bytes % 128 != 0
              ? launch_cut<true>(p, tiles_n, grid, blocks, stream)
              : launch_cut<false>(p, tiles_n, grid, blocks, stream);

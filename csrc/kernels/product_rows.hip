@@ -297,12 +297,10 @@ hipError_t launch(const ProductArgs& p, hipStream_t stream) {
   const int tiles_n = (p.n + NF * 16 - 1) / (NF * 16);
   const long long blocks = static_cast<long long>(tiles_m) * tiles_n +
                            (p.zero_rest ? kZeroBlocks : 0);
-  if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
   constexpr int lds = W * MF * NF * 64 * 16;
   static_assert(lds <= 65536, "more LDS than a launch may ask for");
-  return launch_kernel(&product_rows_kernel<MODE, EPI, MF, NF, W>,
-                       dim3(static_cast<unsigned>(blocks)), dim3(64 * W), lds,
-                       stream, p, tiles_m, tiles_n);
+  return launch_tiles(&product_rows_kernel<MODE, EPI, MF, NF, W>, blocks,
+                      64 * W, lds, stream, p, tiles_m, tiles_n);
 }
 
 // fragments of 16 columns over all row tiles of MF fragments

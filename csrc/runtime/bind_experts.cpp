@@ -124,8 +124,7 @@ void bind_experts(py::module_& m) {
          int rows_a, int rows_c, int n, int row_bytes, int experts,
          int epilogue, bool zero_rest, int cus, addr_t partial,
          addr_t stream) {
-        check_hip(experts_prepare(), "experts_prepare");
-        ProductArgs p;
+        ProductArgs p{};
         p.cus = cus;
         p.partial = ptr<float>(partial);
         p.a = ptr<const uint8_t>(a);
@@ -144,6 +143,13 @@ void bind_experts(py::module_& m) {
         p.experts = experts;
         p.epilogue = epilogue;
         p.zero_rest = zero_rest;
+        p.dry = true;
+        if (launch_product(p, nullptr) == hipErrorInvalidConfiguration)
+          throw py::value_error(
+              "a product of so many experts and columns has more tiles than "
+              "one launch takes (2^32 threads): split the columns");
+        p.dry = false;
+        check_hip(experts_prepare(), "experts_prepare");
         check_hip(launch_product(p, stream_of(stream)), "product");
       },
       py::arg("a"), py::arg("a_scales"), py::arg("b"), py::arg("b_scales"),

@@ -417,6 +417,26 @@ def test_only_the_kernels_that_calls_reach_are_built():
     assert b'product_tile_kernelILi1ELi2E' in built
 
 
+@pytest.mark.parametrize('mx,rows,num,n,row_bytes', [
+    # few rows, with one wave a workgroup and with more
+    (True, 131072, 65536, 32768, 64), (False, 65536, 65536, 16384, 4096),
+    (True, 786432, 65536, 65536, 2048),
+    # 256x256 tiles, in one group and in many
+    (False, 0x7f000000, 1, 1 << 20, 2048),
+    (True, 0x7f000000, 65536, 1 << 20, 192),
+    # 128x128 tiles (weights past 32-bit offsets)
+    (False, 1 << 24, 1, 1 << 24, 1024)])
+def test_more_tiles_than_a_launch_takes_are_refused(mx, rows, num, n,
+                                                    row_bytes):
+    """A grid has fewer than 2^32 threads: an error before anything runs."""
+    if not native.extension_candidates():
+        pytest.skip('the extension is not built')
+    mod = native.load()
+    with pytest.raises(ValueError, match='more tiles than one launch'):
+        mod.product(0, 16 if mx else 0, 0, 16 if mx else 0, 0, 0, 0, 16, 0,
+                    rows, rows, n, row_bytes, num, 0, True, 256, 0, 0)
+
+
 def test_dual_tensors_are_refused(host):
     """A tangent would be lost without a word."""
     forward = torch.autograd.forward_ad
