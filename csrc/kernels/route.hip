@@ -423,9 +423,8 @@ constexpr int kCombineThreads = 256;
 __global__ __launch_bounds__(kCombineThreads) void combine_kernel(
     const uint16_t* __restrict__ y, const int* __restrict__ positions,
     const float* __restrict__ weights, const uint16_t* residual,
-    uint16_t* out, int k, int rows, int width) {
+    uint16_t* out, int k, int rows, int width, int chunks) {
   const int t = blockIdx.x;
-  const int chunks = width / 8;
   const int c = blockIdx.y * kCombineThreads + threadIdx.x;
   if (c >= chunks) return;
   const size_t at = static_cast<size_t>(t) * width + c * 8;
@@ -481,21 +480,28 @@ hipError_t launch_combine(const uint16_t* y, const int* positions,
   if (tokens < 0 || k < 1 || rows < 0 || width < 8 || width % 8 != 0)
     return hipErrorInvalidValue;
   if (tokens == 0) return hipSuccess;
-  // (a grid has fewer than 2^32 threads along one axis)
-  constexpr int kPart = 1 << 23;
-  for (int first = 0;; first += kPart) {
+  // (a grid has fewer than 2^32 threads along its first axis, and 2^16
+  // workgroups along its second)
+  constexpr int kPart = 1 << 23, kPartChunks = 65535 * kCombineThreads;
+  for (int first = 0; first < tokens; first += kPart) {
     const int count = tokens - first < kPart ? tokens - first : kPart;
     const size_t slot = static_cast<size_t>(first) * k;
-    const size_t at = static_cast<size_t>(first) * width;
-    const dim3 grid(count,
-                    (width / 8 + kCombineThreads - 1) / kCombineThreads);
-    const hipError_t err = launch_kernel(
-        &combine_kernel, grid, dim3(kCombineThreads), 0, stream, y,
-        positions + slot, weights + slot,
-        residual != nullptr ? residual + at : nullptr, out + at, k, rows,
-        width);
-    if (err != hipSuccess || first + count == tokens) return err;
+    for (int chunk = 0; chunk < width / 8; chunk += kPartChunks) {
+      const int left = width / 8 - chunk;
+      const int chunks = left < kPartChunks ? left : kPartChunks;
+      const size_t col = static_cast<size_t>(chunk) * 8;
+      const size_t at = static_cast<size_t>(first) * width + col;
+      const dim3 grid(count,
+                      (chunks + kCombineThreads - 1) / kCombineThreads);
+      const hipError_t err = launch_kernel(
+          &combine_kernel, grid, dim3(kCombineThreads), 0, stream, y + col,
+          positions + slot, weights + slot,
+          residual != nullptr ? residual + at : nullptr, out + at, k, rows,
+          width, chunks);
+      if (err != hipSuccess) return err;
+    }
   }
+  return hipSuccess;
 }
 
 }  // namespace kiosk

@@ -1085,6 +1085,18 @@ def test_calls_on_two_streams_at_once(mx):
 
 
 @gpu
+def test_combine_of_a_wide_row():
+    """More stretches of columns than 16 bits count."""
+    width = (1 << 27) + 2048 + 8
+    y = torch.ones(1, width, dtype=BF16, device='cuda')
+    y[0, 1 << 27:] = 3
+    positions = torch.zeros(1, 1, dtype=torch.int32, device='cuda')
+    out = experts.combine(y, positions, torch.full((1, 1), 0.5,
+                                                   device='cuda'))
+    assert torch.equal(out, y / 2)
+
+
+@gpu
 @pytest.mark.parametrize('m,n,k', [(4, 512, 512), (512, 512, 1024),
                                    (1500, 1024, 4096)])
 def test_a_bf16_residual_is_refused_by_the_binding(m, n, k):
