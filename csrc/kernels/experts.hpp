@@ -76,6 +76,8 @@ struct ProductArgs {
 // Bytes of fp32 workspace that speed the product up (0: none is used).  Only
 // the sizes, `cus` and whether scales, offsets and rows are null matter.
 size_t product_workspace(const ProductArgs& args);
+// The kernel that such a product runs on: "rows", "tile128" or "tile256".
+const char* product_kernel(const ProductArgs& args);
 // hipErrorInvalidConfiguration: more tiles than one launch takes.
 hipError_t launch_product(const ProductArgs& args, hipStream_t stream);
 hipError_t experts_prepare();   // load the code objects, raise LDS limits

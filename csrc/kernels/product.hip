@@ -303,6 +303,11 @@ size_t product_workspace(const ProductArgs& p) {
   return pick(p) == k256 ? product256_workspace(p) : 0;
 }
 
+const char* product_kernel(const ProductArgs& p) {
+  const Variant v = pick(p);
+  return v == kRows ? "rows" : v == kTile ? "tile128" : "tile256";
+}
+
 hipError_t launch_product(const ProductArgs& p, hipStream_t stream) {
   // (an empty tensor has no address: nothing below holds for it)
   if (p.rows_c == 0) return hipSuccess;

@@ -19,6 +19,26 @@ hipStream_t stream_of(addr_t s) {
   return reinterpret_cast<hipStream_t>(static_cast<uintptr_t>(s));
 }
 
+// A product's sizes without its operands; `grouped`, `gather`: offsets and
+// rows are given.
+ProductArgs product_sizes(bool mx, bool grouped, bool gather, int rows_a,
+                          int rows_c, int n, int row_bytes, int experts,
+                          int cus) {
+  static const uint8_t some = 0;
+  static const int one = 0;
+  ProductArgs p{};
+  p.a_scales = p.b_scales = mx ? &some : nullptr;
+  p.offsets = grouped ? &one : nullptr;
+  p.rows = gather ? &one : nullptr;
+  p.rows_a = rows_a;
+  p.rows_c = rows_c;
+  p.n = n;
+  p.row_bytes = row_bytes;
+  p.experts = experts;
+  p.cus = cus;
+  return p;
+}
+
 }  // namespace
 
 void bind_experts(py::module_& m) {
@@ -94,29 +114,19 @@ void bind_experts(py::module_& m) {
       py::arg("codes"), py::arg("scales"), py::arg("out"), py::arg("bf16"),
       py::arg("n"), py::arg("stream"),
       py::call_guard<py::gil_scoped_release>());
-  // bytes of workspace for such a product; `grouped`, `gather`: offsets and
-  // rows are given
-  m.def(
-      "product_workspace",
-      [](bool mx, bool grouped, bool gather, int rows_a, int rows_c, int n,
-         int row_bytes, int experts, int cus) {
-        static const uint8_t some = 0;
-        static const int one = 0;
-        ProductArgs p{};
-        p.a_scales = p.b_scales = mx ? &some : nullptr;
-        p.offsets = grouped ? &one : nullptr;
-        p.rows = gather ? &one : nullptr;
-        p.rows_a = rows_a;
-        p.rows_c = rows_c;
-        p.n = n;
-        p.row_bytes = row_bytes;
-        p.experts = experts;
-        p.cus = cus;
-        return product_workspace(p);
-      },
-      py::arg("mx"), py::arg("grouped"), py::arg("gather"),
-      py::arg("rows_a"), py::arg("rows_c"), py::arg("n"),
-      py::arg("row_bytes"), py::arg("experts"), py::arg("cus"));
+  // bytes of workspace for such a product, and the kernel that it runs on
+  m.def("product_workspace", [](bool mx, bool grouped, bool gather, int rows_a,
+                                int rows_c, int n, int row_bytes, int experts,
+                                int cus) {
+    return product_workspace(product_sizes(mx, grouped, gather, rows_a, rows_c,
+                                           n, row_bytes, experts, cus));
+  });
+  m.def("product_kernel", [](bool mx, bool grouped, bool gather, int rows_a,
+                             int rows_c, int n, int row_bytes, int experts,
+                             int cus) {
+    return product_kernel(product_sizes(mx, grouped, gather, rows_a, rows_c, n,
+                                        row_bytes, experts, cus));
+  });
   m.def(
       "product",
       [](addr_t a, addr_t a_scales, addr_t b, addr_t b_scales, addr_t c,

@@ -1084,6 +1084,197 @@ def test_calls_on_two_streams_at_once(mx):
         assert torch.equal(out, want)
 
 
+def kernel_of(a, b, rows=None, grouped=True):
+    """The kernel that a product runs on."""
+    mx = isinstance(a, mxfp4.Mxfp4)
+    part_a, part_b = (a.codes, b.codes) if mx else (a, b)
+    return native.load().product_kernel(
+        mx, grouped, rows is not None, part_a.shape[0],
+        part_a.shape[0] if rows is None else rows.numel(), part_b.shape[-2],
+        part_a.shape[1] * part_a.element_size(),
+        part_b.shape[0] if grouped else 1,
+        native.load().device_cus(part_a.device.index))
+
+
+def whole_mx(*shape, seed):
+    """Multiples of a half up to 24, every code under three scales."""
+    q = random_mx(*shape, seed=seed)
+    g = torch.Generator(device='cuda').manual_seed(seed + 1)
+    q.scales[:] = torch.randint(127, 130, q.scales.shape, generator=g,
+                                device='cuda', dtype=torch.uint8)
+    return q
+
+
+def whole_bf16(*shape, seed):
+    """Whole numbers up to 56, a power of two for every 32 of them."""
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    x = torch.randint(-7, 8, shape[:-1] + (shape[-1] // 32, 32), generator=g,
+                      device='cuda')
+    e = torch.randint(0, 4, shape[:-1] + (shape[-1] // 32, 1), generator=g,
+                      device='cuda')
+    return (x << e).view(shape).to(BF16)
+
+
+def exact_product(a, b, bias=None, residual=None):
+    """The product of whole numbers, rounded once.  All terms are multiples
+    of a quarter and their magnitudes add up to less than 2^22: every sum of
+    some of them is an fp32 number, in whichever order they are added."""
+    y = a @ b.t()
+    size = a.abs() @ b.abs().t()
+    for part in (bias, residual):
+        if part is not None:
+            y, size = y + part.double(), size + part.double().abs()
+    assert float(size.max()) < 2.0 ** 22
+    assert torch.equal(y.float().double(), y)
+    return y.float().to(BF16)
+
+
+# kernel, rows, experts, n, K of MXFP4, K of bf16.  Rows of MXFP4 end with
+# half a step of 128 bytes wherever K is no multiple of 256; of the few-rows
+# kernel with 64, 128 or 192 bytes behind the last 256
+EXACT = [
+    # few rows, a wave for every quarter of the row, many turns each
+    ('rows', 3, 1, 128, 16384, 8192), ('rows', 17, 1, 96, 32768, 8256),
+    ('rows', 50, 2, 272, 16768, 4160),
+    # one to four rows a group, many columns: rows of 2 KiB and more
+    ('rows', 8, 8, 2048, 3968, 960), ('rows', 4, 4, 4096, 8576, 2112),
+    # five and more: four waves, one wave
+    ('rows', 24, 4, 4096, 8448, 2112), ('rows', 128, 16, 4096, 3968, 960),
+    ('rows', 100, 4, 4096, 8576, 2112), ('rows', 100, 4, 9632, 2176, 576),
+    # 128 x 128 tiles: at most one for each CU, two
+    ('tile128', 300, 1, 528, 2176, 576), ('tile128', 900, 5, 528, 1920, 512),
+    ('tile128', 900, 5, 4096, 4096, 1024),
+    # 256 x 256 tiles: slices of few tiles and of a last round, none
+    ('tile256', 300, 2, 528, 16768, 4160), ('tile256', 300, 1, 272, 8576,
+                                            2112),
+    ('tile256', 2000, 3, 4624, 8448, 2112), ('tile256', 1100, 8, 8192, 1152,
+                                             320),
+    ('tile256', 5000, 7, 2064, 8320, 2240)]
+
+
+@gpu
+@pytest.mark.parametrize('mx', [False, True])
+@pytest.mark.parametrize('kernel,rows,num,n,k_mx,k_bf16', EXACT)
+def test_products_of_whole_numbers_are_exact(kernel, rows, num, n, k_mx,
+                                             k_bf16, mx):
+    """A block of the inner dimension that is lost, read twice or scaled by
+    its neighbour's scale shows as a wrong number."""
+    k, make = (k_mx, whole_mx) if mx else (k_bf16, whole_bf16)
+    a, b = make(rows, k, seed=rows), make(num, n, k, seed=n)
+    offsets = cut(rows, num, 1)
+    assert kernel_of(a, b) == kernel
+    bias = torch.randint(-99, 100, (num, n), device='cuda',
+                         generator=torch.Generator('cuda').manual_seed(
+                             5)).float()
+    out = experts.grouped_gemm(a, b, offsets, bias, 'bias')
+    va, vb = (values_of(a), values_of(b)) if mx else (a.double(), b.double())
+    bounds = offsets.tolist()
+    for e in range(num):
+        lo, hi = bounds[e], bounds[e + 1]
+        if lo < hi:
+            assert torch.equal(out[lo:hi], exact_product(va[lo:hi], vb[e],
+                                                         bias[e])), e
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(2))
+    order = order.to(torch.int32).cuda()
+    assert kernel_of(a, b, order) == kernel
+    out = experts.grouped_gemm(a, b, offsets, rows=order)
+    for e in range(num):
+        lo, hi = bounds[e], bounds[e + 1]
+        if lo < hi:
+            assert torch.equal(out[lo:hi], exact_product(
+                va[order[lo:hi].long()], vb[e])), e
+
+
+@gpu
+@pytest.mark.parametrize('kernel,m,n,k', [
+    ('rows', 3, 128, 16384), ('rows', 1, 4096, 16768),
+    ('rows', 30, 4096, 8576), ('tile128', 300, 528, 2176),
+    ('tile128', 900, 4096, 4096), ('tile256', 300, 528, 16768),
+    ('tile256', 1000, 1040, 8320), ('tile256', 2600, 8208, 1152)])
+def test_mxfp4_products_with_a_residual_are_exact(kernel, m, n, k):
+    a, b = whole_mx(m, k, seed=m), whole_mx(n, k, seed=n)
+    assert kernel_of(a, b, grouped=False) == kernel
+    g = torch.Generator(device='cuda').manual_seed(3)
+    bias = torch.randint(-99, 100, (n,), generator=g, device='cuda').float()
+    res = torch.randint(-99, 100, (m, n), generator=g, device='cuda').to(BF16)
+    want = exact_product(values_of(a), values_of(b), bias, res)
+    assert torch.equal(mxfp4.gemm(a, b, bias, res, 'residual'), want)
+    assert torch.equal(mxfp4.gemm(a, b, bias, res, 'residual', out=res), want)
+
+
+@gpu
+@pytest.mark.parametrize('n,k', [(32, 4096), (16400, 4096), (65552, 1024)])
+def test_few_rows_out_of_a_large_input_are_exact(n, k):
+    """Groups of up to 64 rows, gathered from more than 4 GiB."""
+    rows = (1 << 32) // (2 * k) + 7
+    a = torch.zeros(rows, k, dtype=BF16, device='cuda')
+    at = torch.cat([torch.arange(30), torch.arange(rows - 30, rows)])
+    a[at.cuda()] = whole_bf16(60, k, seed=1)
+    b = whole_bf16(1, n, k, seed=2)
+    index = at.to(torch.int32).cuda()
+    assert kernel_of(a, b, index) == 'rows'
+    out = experts.grouped_gemm(a, b, torch.tensor(
+        [0, 60], dtype=torch.int32, device='cuda'), rows=index)
+    assert torch.equal(out, exact_product(a[at.cuda()].double(),
+                                          b[0].double()))
+
+
+@gpu
+@pytest.mark.parametrize('mx', [False, True])
+@pytest.mark.parametrize('rows,n', [(700, 272), (700, 16400)])
+def test_rows_outside_the_groups_of_large_tiles(rows, n, mx):
+    """256 x 256 tiles, sliced and whole: zero in a new result, as they were
+    in ``out``; NaN there, or in an empty group's weights, reaches no other
+    row."""
+    num, k = 4, (10240 if mx else 2560) if n < 1024 else (640 if mx else 320)
+    a, b = rand(rows, k, seed=1), rand(num, n, k, seed=2)
+    a[:3] = math.nan
+    a[rows - 5:] = math.nan
+    b[3] = math.nan                                  # its group is empty
+    offsets = torch.tensor([3, 9, 9, rows - 5, rows - 5], dtype=torch.int32,
+                           device='cuda')
+    if mx:
+        a, b = mxfp4.quantize(a), mxfp4.quantize(b)
+    assert kernel_of(a, b) == 'tile256'
+    assert (experts.workspace_bytes(a, b) > 0) is (n < 1024)
+    out = experts.grouped_gemm(a, b, offsets)
+    assert (out[:3] == 0).all() and (out[rows - 5:] == 0).all()
+    assert out[3:rows - 5].isfinite().all()
+    kept = torch.full((rows, n), 7.0, dtype=BF16, device='cuda')
+    assert experts.grouped_gemm(a, b, offsets, out=kept) is kept
+    assert (kept[:3] == 7).all() and (kept[rows - 5:] == 7).all()
+    assert torch.equal(kept[3:rows - 5], out[3:rows - 5])
+    none = torch.zeros(num + 1, dtype=torch.int32, device='cuda')
+    assert (experts.grouped_gemm(a, b, none) == 0).all()
+    kept.fill_(7)
+    assert (experts.grouped_gemm(a, b, none, out=kept) == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize('mx', [False, True])
+@pytest.mark.parametrize('kernel,rows,n,k', [
+    ('rows', 30, 256, 8576), ('tile256', 300, 256, 10240),
+    ('tile256', 300, 65552, 640)])
+def test_one_row_does_not_depend_on_its_neighbours_in_any_kernel(
+        kernel, rows, n, k, mx):
+    """A row's result is the same wherever the batch puts it within one size,
+    and a NaN row stays alone: few rows, and 256 x 256 tiles in slices and
+    whole ones (the 128 x 128 ones have a test of their own)."""
+    a, b = rand(rows, k, seed=1), rand(1, n, k, seed=2)
+    a[17] = math.nan
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device='cuda')
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(1))
+    order = order.to(torch.int32).cuda()
+    if mx:
+        a, b = mxfp4.quantize(a), mxfp4.quantize(b)
+    assert kernel_of(a, b) == kernel_of(a, b, order) == kernel
+    out = experts.grouped_gemm(a, b, offsets)
+    assert out[17].isnan().all() and int(out.isnan().sum()) == n
+    moved = experts.grouped_gemm(a, b, offsets, rows=order)
+    assert torch.equal(moved.view(torch.int16),
+                       out[order.long()].view(torch.int16))
+
+
 @gpu
 def test_combine_of_a_wide_row():
     """More stretches of columns than 16 bits count."""
