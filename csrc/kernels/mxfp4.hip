@@ -13,8 +13,8 @@
 // maximum is taken over the block's bit patterns (as integers: a NaN stays
 // the largest) with two lane exchanges in the VALU, and the conversion
 // instruction, which divides by the scale, makes two codes at a time.  16384 x
-// 4096 bf16: 32 us, 5.4 TB/s (50 with the borders compared one by one); back
-// again 28.5 us.
+// 4096 bf16: 31-34 us, 5.0-5.5 TB/s (50 with the borders compared one by one);
+// back again 28.5 us.
 #include "common.hpp"
 #include "experts.hpp"
 #include "kernels.hpp"

@@ -1,8 +1,9 @@
 // The bf16 product's 256 x 256 tile for groups of many rows (contract:
 // product.hip; division of the work and LDS ring: product256.hpp).
 //
-// Bound by the card's power as the MXFP4 one: 4096 x 4096 x 8192 takes 184 us
-// (1.5 PFLOP/s), 142 on zeros; a large library product reaches 1.6 PFLOP/s.
+// Bound by the card's power: 4096 x 4096 x 8192 takes 187 us (1.5 PFLOP/s), 144
+// on zeros (of rows of 64 KiB 760 and 743: there it is memory); a large library
+// product reaches 1.6 PFLOP/s.
 //
 // Four waves of 128 x 128 outputs (128 x 64 of a tile of 128 rows), the
 // accumulators in AGPRs.  v_mfma_f32_16x16x32_bf16: the 32 x 32 one, with half

@@ -1,9 +1,9 @@
 // The MXFP4 product's 256 x 256 tile for groups of many rows (contract:
 // product.hip; division of the work and LDS ring: product256.hpp).
 //
-// Bound by the card's power: 4096 x 4096 x 16384 takes 121 us (4.5 PFLOP/s; the
-// clock falls to 1.8 GHz) and, with the same instructions on zeros, 89 us.
-// Besides, a tile costs some 10 us that no other one's work covers (it has
+// Bound by the card's power and by its loads: 4096 x 4096 x 16384 takes 123 us
+// (4.5 PFLOP/s; the clock falls to 1.8 GHz), with the same instructions on
+// zeros 88 us, without LDS reads and loads in the loop 94.  Besides, a tile costs some 10 us that no other one's work covers (it has
 // the CU's LDS to itself): the first loads and the stores.
 //
 // Four waves of 128 x 128 outputs (128 x 64 of a tile of 128 rows), the

@@ -18,8 +18,8 @@
 // Choosing is what takes time, and it is a chain: k times a maximum over the
 // experts.  Up to 256 experts lie on 16 lanes, so that a wave works on four
 // tokens at once and a maximum is four row rotations in the VALU.  16384
-// tokens, 128 experts, k = 8, bf16: 9 us and 7 for the second launch (one token
-// a wave: 84 in all); one token: 4 us.
+// tokens, 128 experts, k = 8, bf16: 9.6 us and 7-8 for the second launch (one
+// token a wave: 84 in all); one token: 4 us.
 //
 // The sum is bound by memory: 8192 tokens of 4 rows of 4096 in 66 us, 5.6
 // TB/s.
