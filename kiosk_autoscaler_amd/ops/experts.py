@@ -74,7 +74,7 @@ def route(logits, k, renormalize=True, out=None):
     :class:`Plan` to write to."""
     import torch
     device = checks.tensor(logits, 'logits',
-                           (torch.bfloat16, torch.float32), dims=2, align=4)
+                           (torch.bfloat16, torch.float32), dims=2, align=2)
     mod = native.load()
     tokens, experts = logits.shape
     k = int(k)

@@ -225,6 +225,15 @@ def test_route_refuses(host, logits, k, match):
         experts.route(logits, k)
 
 
+def test_route_takes_any_row_of_logits(host):
+    """Rows of an odd number of bf16 logits start at odd multiples of two
+    bytes."""
+    logits = zeros(4, 5)
+    for first in range(4):
+        with pytest.raises(AssertionError, match='launched'):
+            experts.route(logits[first:], 2)
+
+
 def test_route_refuses_a_wrong_plan(host):
     logits = zeros(200, 8)
     good = experts.empty_plan(200, 8, 2, 'cpu')
@@ -522,6 +531,32 @@ def test_route_of_infinite_and_nan_logits(tokens, renormalize):
     assert bool(got.weights[:2].isnan().all())
     assert torch.equal(got.experts[2:], want.experts[2:])
     assert torch.equal(got.weights[2:], want.weights[2:])
+
+
+@gpu
+@pytest.mark.parametrize('num,k', [(5, 2), (27, 4), (301, 3)])
+def test_route_of_rows_at_odd_addresses(num, k):
+    logits = rand(700, num, seed=7)
+    for first in (1, 2, 3):
+        part = logits[first:]
+        got, want = experts.route(part, k), experts.route(part.clone(), k)
+        for a, b in zip(got[:5], want[:5]):
+            assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize('kernel,m,n,k', [
+    ('rows', 5, 272, 16768), ('rows', 30, 4096, 2176),
+    ('tile128', 300, 528, 2176), ('tile256', 300, 528, 8576)])
+def test_mxfp4_products_of_scales_at_any_word(kernel, m, n, k):
+    """Scale rows of an odd number of words, from the second row on."""
+    a, b = whole_mx(m + 1, k, seed=m), whole_mx(n + 1, k, seed=n)
+    part_a, part_b = (mxfp4.Mxfp4(q.codes[1:], q.scales[1:])
+                      for q in (a, b))
+    assert part_b.scales.data_ptr() % 8
+    assert kernel_of(part_a, part_b, grouped=False) == kernel
+    assert torch.equal(mxfp4.gemm(part_a, part_b), exact_product(
+        values_of(part_a), values_of(part_b)))
 
 
 @gpu
